@@ -8,7 +8,6 @@ this library makes.  ``exact`` is the same in 64 bits, written apart from the pl
 """
 from __future__ import annotations
 
-import functools
 import math
 import os
 import sys
@@ -196,7 +195,6 @@ def run(state):
     return {"append": _append_pass, "route": _route_pass, "attend": _attend_pass}[state["case"]["op"]](state)
 
 
-@functools.cache                                         # a program imports once
 def _library():
     package = os.path.join(os.getcwd(), "relation-lm_b200")
     if package not in sys.path:
