@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(kBaThreads) block_attention_rows_kernel(const 
     __syncthreads();
 
     // 16 keys at a time: first the kept blocks', each block from its own first row, then the window's
-    const int per_block = (a.block_size + 15) >> 4;
+    const int per_block = (min(a.block_size, start) + 15) >> 4;      // a block's rows from the window on are the window's
     const int block_chunks = n_kept * per_block;
     const int chunks = block_chunks + ((t - start + 16) >> 4);
     const int step = kBaWarps * a.splits;
@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(kBaThreads, D != 64 ? 1 : kFpHeads == 1 ? 7 : 
     if (warp == 0) keep_blocks(index, first, a.top, a.block_size, start, kept, &n_kept);
     const float scale = a.flip ? -a.scale_log2 : a.scale_log2;
     __syncthreads();
-    const int per_block = (a.block_size + kFpChunk - 1) / kFpChunk;
+    const int per_block = (min(a.block_size, start) + kFpChunk - 1) / kFpChunk;
     const int block_chunks = n_kept * per_block;
     const int chunks = block_chunks + (t - start + kFpChunk) / kFpChunk;
     const unsigned char* keys = a.key_cache + seq * a.k_seq + kv * a.k_head + 16 * part;
@@ -577,7 +577,7 @@ int attention_args(AttentionArgs& a, const int64_t* position, const int32_t* row
     a.kv_heads = kv_heads;
     a.group = heads / kv_heads;
     a.top = top_blocks;
-    a.block_size = block_size;
+    a.block_size = block_size < max_t ? block_size : max_t;      // the first block is all that begins before a window
     a.window = local_window < max_t ? local_window : max_t;      // no row has more before it
     return RLM_OK;
 }
@@ -641,7 +641,7 @@ extern "C" int rlm_block_attention(const void* query, const void* key_cache, con
     // a row's keys over a cluster of CTAs, while the launch leaves SMs idle and every warp keeps a pass of 16 keys (beyond
     // that a cluster's joins cost more than the idle end of the launch: 512 CTAs of 1536 keys 69 us, as 1024 84)
     const int64_t ctas = static_cast<int64_t>(n_rows) * kv_heads * a.head_tiles;
-    const int64_t passes = (static_cast<int64_t>(top_blocks) * ((block_size + 15) / 16) + (a.window + 15) / 16 + kBaWarps - 1) / kBaWarps;
+    const int64_t passes = (static_cast<int64_t>(top_blocks) * ((a.block_size + 15) / 16) + (a.window + 15) / 16 + kBaWarps - 1) / kBaWarps;
     a.splits = 1;
     while (a.splits < kBaMaxSplit && ctas * a.splits * 2 <= 2 * sm_count() && passes >= 2 * a.splits) a.splits *= 2;
     if (ctas * a.splits > 0x7fffffff) {

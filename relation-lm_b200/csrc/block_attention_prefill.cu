@@ -371,7 +371,9 @@ __global__ void __launch_bounds__(kBpThreads) block_attention_tiles_kernel(const
 
     const unsigned char* key_rows = a.key_cache + g.seq * a.k_seq + kv * a.k_head;
     const unsigned char* value_rows = a.value_cache + g.seq * a.v_seq + kv * a.v_head;
-    const int at = tile.block * a.block_size, cached = min(a.block_size, a.rows.max_t - at);
+    const int at = tile.block * a.block_size;
+    // rows of the block before the last window of the segment; no entry sees more
+    const int cached = min(a.block_size, g.t0 + g.rows - a.window - at);
     request_rows<D, kKeys>(keys, key_rows, a.k_row, at, cached);
     request_rows<D, kKeys>(values, value_rows, a.v_row, at, cached);
     for (int e = threadIdx.x; e < tile.entries; e += kBpThreads) {
@@ -414,7 +416,7 @@ __global__ void __launch_bounds__(kBpThreads) block_attention_tiles_kernel(const
         request_queries(strip + kBpWarps, (j + 1) & 1);
         Running<D> run;
         run.clear();
-        for (int o = 0; o < a.block_size; o += kKeys) {
+        for (int o = 0; o < cached; o += kKeys) {
             if (!one_chunk && (o > 0 || j > 0)) {
                 __syncthreads();
                 request_rows<D, kKeys>(keys, key_rows, a.k_row, at + o, cached - o);

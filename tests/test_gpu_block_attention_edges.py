@@ -1,0 +1,80 @@
+"""Attention over router-chosen blocks at its borders: sizes, layouts, memory and values that ordinary calls do not reach."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import block_attention_util as plain
+from relation_lm.kernels import block_attention as ba
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+HALF_TYPES = (torch.bfloat16, torch.float16)
+
+
+def random(g, *shape, dtype=torch.float32, scale=1.0):
+    return (torch.randn(*shape, generator=g) * scale).to(dtype)
+
+
+def within(got, want, bound, what=""):
+    error = (got.double().cpu() - want).abs()
+    assert bool((error <= bound).all()), (what, float((error - bound).max()))
+
+
+def status_clear():
+    from relation_lm.kernels import _abi
+
+    assert _abi.read_status() == 0
+
+
+def check_rows(some, at, q, k_cache, v_cache, index, out, lse, block_size, window, scale):
+    """Rows ``some`` of a call against the 64-bit form; ``index`` is [rows, kv_heads, places]."""
+    for i in some:
+        b, t = at[i]
+        want, want_lse, bound, lse_bound = plain.attend(q[i].cpu(), k_cache[b].cpu(), v_cache[b].cpu(), index[i].cpu(), t, block_size,
+                                                        window, scale)
+        within(out[i], want, bound, (i, b, t))
+        empty = want_lse == -math.inf
+        assert bool((lse[i].cpu()[empty] == -math.inf).all())
+        within(lse[i].cpu()[~empty], want_lse[~empty], lse_bound[~empty], "lse")
+
+
+# ---------------------------------------------------------------------------- blocks longer than the cache
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("form", ("decode", "rows", "prefill"))
+@pytest.mark.parametrize("context,window", [(9, 2), (200, 30)])
+@pytest.mark.parametrize("block_size", ("one more", 1 << 20, "most"))
+def test_blocks_longer_than_the_cache(dtype, form, context, window, block_size):
+    # the first block is then all that lies before the window; the largest size that the entry point takes among them
+    block_size = {"one more": context + 1, "most": 0x7fffffff - context}.get(block_size, block_size)
+    g = torch.Generator().manual_seed(context)
+    at = [(b, context - 1) for b in range(2)] if form == "decode" else plain.places(form, 2, min(2 * context, 25), context, context)
+    n = len(at)
+    q = random(g, n, 4, 64, dtype=dtype)
+    k_cache, v_cache = (random(g, 2, context, 2, 64, dtype=dtype) for _ in range(2))
+    index = torch.tensor([0, 1, 0, -1], dtype=torch.int32).expand(n, 2, 4)
+    call = {"decode": ba.block_attention, "rows": ba.block_attention_rows, "prefill": ba.block_attention_prefill}[form]
+    out, lse = call(q.cuda(), k_cache.cuda(), v_cache.cuda(), index.cuda(), *plain.where(form, at, context), block_size, window, 0.125)
+    check_rows(range(0, n, 1 + n // 40), at, q, k_cache, v_cache, index, out, lse, block_size, window, 0.125)
+    status_clear()
+
+
+@pytest.mark.parametrize("dtype", HALF_TYPES)
+@pytest.mark.parametrize("width", (64, 96))
+@pytest.mark.parametrize("block_size,spare", [(500, 0), (601, 0), (1 << 20, 70), (0x7fffffff - 671, 70)])
+def test_blocks_longer_than_whole_sequences(dtype, width, block_size, spare):
+    length, window = 601, 40
+    g = torch.Generator().manual_seed(width)
+    at = plain.places("prefill", 2, 0, 0, length)
+    q = random(g, len(at), 4, width, dtype=dtype)
+    k_cache, v_cache = (random(g, 2, length + spare, 2, width, dtype=dtype) for _ in range(2))
+    k_cache[:, length:], v_cache[:, length:] = math.nan, math.inf            # nothing has been written there yet
+    index = torch.randint(-1, 3, (len(at), 2, 3), generator=g, dtype=torch.int32)
+    out, lse = ba.block_attention_prefill(q.cuda(), k_cache.cuda(), v_cache.cuda(), index.cuda(), length, block_size, window, 0.125)
+    check_rows([0, 1, window, 300, 600, 601, 777, 1200, 1201], at, q, k_cache, v_cache, index, out, lse, block_size, window, 0.125)
+    status_clear()
