@@ -25,6 +25,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <initializer_list>
 #include <mutex>
 #include <optional>
@@ -1074,6 +1075,51 @@ bool share_bytes(const Tensor& a, const Tensor& b) {
     return x.first < y.second && y.first < x.second;
 }
 
+// Whether two tensors of one dtype have a byte in common: whether the distance between their first elements is a sum of
+// whole steps within the extents of both.  The steps are tried from the longest on, each as often as leaves a rest that the
+// shorter ones can make up.  The strides of views of one buffer nest, which leaves one or two choices a dimension; a search
+// that does not end soon counts as common memory.
+bool share_elements(const Tensor& a, const Tensor& b) {
+    if (!share_bytes(a, b)) return false;
+    struct Step { int64_t bytes, least, most, rest_least, rest_most; };
+    std::vector<Step> steps;
+    const int64_t size = static_cast<int64_t>(a.element_size());
+    auto add = [&](int64_t bytes, int64_t least, int64_t most) {
+        if (bytes == 0 || least == most) return;
+        for (Step& s : steps)
+            if (s.bytes == bytes) {
+                s.least += least;
+                s.most += most;
+                return;
+            }
+        steps.push_back(Step{bytes, least, most, 0, 0});
+    };
+    for (int64_t d = 0; d < a.dim(); ++d) add(a.stride(d) * size, 0, a.size(d) - 1);
+    for (int64_t d = 0; d < b.dim(); ++d) add(b.stride(d) * size, 1 - b.size(d), 0);
+    add(1, 1 - size, size - 1);                          // the bytes of an element
+    std::sort(steps.begin(), steps.end(), [](const Step& x, const Step& y) { return x.bytes > y.bytes; });
+    int64_t least = 0, most = 0;
+    for (size_t i = steps.size(); i-- > 0;) {
+        steps[i].rest_least = least;
+        steps[i].rest_most = most;
+        least += steps[i].least * steps[i].bytes;
+        most += steps[i].most * steps[i].bytes;
+    }
+    int budget = 1 << 12;
+    auto floor_div = [](int64_t x, int64_t y) { return x / y - (x % y < 0); };
+    auto reach = [&](auto& self, size_t i, int64_t distance) -> bool {
+        if (--budget < 0) return true;
+        if (i == steps.size()) return distance == 0;
+        const Step& s = steps[i];
+        const int64_t from = std::max(s.least, -floor_div(s.rest_most - distance, s.bytes));
+        const int64_t to = std::min(s.most, floor_div(distance - s.rest_least, s.bytes));
+        for (int64_t n = from; n <= to; ++n)
+            if (self(self, i + 1, distance - n * s.bytes)) return true;
+        return false;
+    };
+    return reach(reach, 0, static_cast<const char*>(b.data_ptr()) - static_cast<const char*>(a.data_ptr()));
+}
+
 void check_caches(const Tensor& key_cache, const Tensor& value_cache, c10::Device device) {
     dense_inside("key_cache", key_cache, 4, device);
     dense_inside("value_cache", value_cache, 4, device);
@@ -1099,8 +1145,7 @@ Tensor append_rotary(const Tensor& query, const Tensor& key, const Tensor& value
                       "query [rows, heads, width], key and value [rows, kv_heads, width] and caches [B, T, kv_heads, width] do not fit");
     for (const Tensor* cache : {&key_cache, &value_cache})
         TORCH_CHECK_VALUE(at::has_internal_overlap(*cache) != at::MemOverlap::Yes, "a cache whose elements share memory cannot be written");
-    TORCH_CHECK_VALUE(at::get_overlap_status(key_cache, value_cache) != at::MemOverlapStatus::Full,
-                      "key_cache and value_cache are the same memory");
+    TORCH_CHECK_VALUE(!share_elements(key_cache, value_cache), "key_cache and value_cache have memory in common");
     for (const Tensor* cache : {&key_cache, &value_cache})
         for (const Named& in : {ARG(query), ARG(key), ARG(value)})
             TORCH_CHECK_VALUE(!share_bytes(*in.t, *cache), in.name, " lies within the memory of a cache that is written");

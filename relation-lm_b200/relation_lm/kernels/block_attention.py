@@ -75,7 +75,8 @@ def rotary_append(query: Tensor, key: Tensor, value: Tensor, key_cache: Tensor, 
     ``[B, T, kv_heads, width]`` (any strides but the innermost), all of one dtype.  ``frequencies`` (fp32 or fp64,
     ``[rotary / 2]``, ``rotary <= width``): component pairs ``(2i, 2i + 1)`` (``interleaved``) or ``(i, i + rotary / 2)`` turn
     by ``position * frequencies[i]`` (worked out in 64 bits) and are multiplied by ``magnitude``; the rest is copied.  A
-    position of a sequence must not occur twice in a call; the inputs must not lie in the caches.
+    position of a sequence must not occur twice in a call; the inputs must not lie in the caches, nor may the caches have an
+    element in common (views of one buffer that lie between one another are fine).
     """
     return _rotary_append(query, key, value, key_cache, value_cache, frequencies, position, interleaved, magnitude)
 

@@ -78,3 +78,43 @@ def test_blocks_longer_than_whole_sequences(dtype, width, block_size, spare):
     out, lse = ba.block_attention_prefill(q.cuda(), k_cache.cuda(), v_cache.cuda(), index.cuda(), length, block_size, window, 0.125)
     check_rows([0, 1, window, 300, 600, 601, 777, 1200, 1201], at, q, k_cache, v_cache, index, out, lse, block_size, window, 0.125)
     status_clear()
+
+
+# ---------------------------------------------------------------------------- caches in one buffer
+
+
+def _pairs_of_views():
+    """(what, key cache, value cache, whether they have an element in common), [2, 6, 2, 32] each."""
+    def buffer(*shape):
+        return torch.randn(*shape, device="cuda").bfloat16()
+
+    three, heads, wide = buffer(3, 6, 2, 32), buffer(2, 6, 3, 32), buffer(2, 6, 2, 48)
+    long, apart, kv = buffer(2, 9, 2, 32), buffer(2, 12, 2, 32), buffer(2, 6, 2, 2, 32)
+    return [("sequences", three[:2], three[1:], True),
+            ("heads", heads[:, :, :2], heads[:, :, 1:], True),
+            ("components", wide[..., :32], wide[..., 16:], True),
+            ("positions", long[:, :6], long[:, 3:], True),
+            ("orders", heads[:, :, :2], heads.view(2, 3, 6, 32)[:, 1:].transpose(1, 2), True),
+            ("the same", three[:2], three[:2], True),
+            ("every other position", apart[:, ::2], apart[:, 1::2], False),
+            ("halves", apart[:, :6], apart[:, 6:], False),
+            ("side by side", kv[:, :, 0], kv[:, :, 1], False),
+            ("heads side by side", kv.view(2, 6, 4, 32)[:, :, :2], kv.view(2, 6, 4, 32)[:, :, 2:], False),
+            ("components side by side", kv.view(2, 6, 2, 64)[..., :32], kv.view(2, 6, 2, 64)[..., 32:], False)]
+
+
+@pytest.mark.parametrize("which", range(11))
+def test_caches_that_overlap_are_refused(which):
+    what, k_cache, v_cache, common = _pairs_of_views()[which]
+    assert k_cache.shape == v_cache.shape == (2, 6, 2, 32)
+    q, k, v = (torch.randn(2, n, 32, device="cuda").bfloat16() for n in (4, 2, 2))
+    f, at = ba.rotary_frequencies(32, device="cuda")[0], torch.tensor(4, device="cuda")
+    if common:
+        with pytest.raises(ValueError, match="in common"):
+            ba.rotary_append(q, k, v, k_cache, v_cache, f, at)
+        with pytest.raises(ValueError, match="in common"):
+            ba.rotary_append(q, k, v, v_cache, k_cache, f, at)
+        return
+    apart = k_cache.clone(), v_cache.clone()
+    out, want = ba.rotary_append(q, k, v, k_cache, v_cache, f, at), ba.rotary_append(q, k, v, *apart, f, at)
+    assert torch.equal(out, want) and torch.equal(k_cache, apart[0]) and torch.equal(v_cache, apart[1]), what
