@@ -564,15 +564,17 @@ int attention_args(AttentionArgs& a, const int64_t* position, const int32_t* row
     }
     const int e = dtype_size(dtype);
     int64_t* const to[8] = {&a.q_row, &a.q_head, &a.k_seq, &a.k_row, &a.k_head, &a.v_seq, &a.v_row, &a.v_head};
+    const int extent[10] = {n_rows, heads, n_seq, max_t, kv_heads, n_seq, max_t, kv_heads, n_rows, kv_heads};
+    auto step = [&](int i) { return extent[i] > 1 ? strides[i] : 0; };       // one of a kind has no step to the next
     for (int i = 0; i < 8; ++i) {
-        *to[i] = strides[i] * e;
+        *to[i] = step(i) * e;
         if (*to[i] % 16 != 0) {
             set_error("block_attention: queries and cache rows must lie on 16-byte boundaries");
             return RLM_ERR_ALIGN;
         }
     }
-    a.i_row = strides[8];
-    a.i_head = strides[9];
+    a.i_row = step(8);
+    a.i_head = step(9);
     a.heads = heads;
     a.kv_heads = kv_heads;
     a.group = heads / kv_heads;

@@ -289,8 +289,9 @@ extern "C" int rlm_rotary_append(const void* query, const void* key, const void*
                              &a.kc_seq, &a.kc_row, &a.kc_head, &a.vc_seq, &a.vc_row, &a.vc_head};
     bool aligned = aligned16(query) && aligned16(key) && aligned16(value) && aligned16(query_out) && aligned16(key_cache) &&
                    aligned16(value_cache);
+    const int extent[12] = {n_rows, heads, n_rows, kv_heads, n_rows, kv_heads, n_seq, max_t, kv_heads, n_seq, max_t, kv_heads};
     for (int i = 0; i < 12; ++i) {
-        *to[i] = strides[i] * e;
+        *to[i] = extent[i] > 1 ? strides[i] * e : 0;     // one of a kind has no step to the next
         aligned = aligned && *to[i] % 16 == 0;
     }
     a.magnitude = magnitude;

@@ -118,3 +118,30 @@ def test_caches_that_overlap_are_refused(which):
     apart = k_cache.clone(), v_cache.clone()
     out, want = ba.rotary_append(q, k, v, k_cache, v_cache, f, at), ba.rotary_append(q, k, v, *apart, f, at)
     assert torch.equal(out, want) and torch.equal(k_cache, apart[0]) and torch.equal(v_cache, apart[1]), what
+
+
+# ---------------------------------------------------------------------------- one row, one sequence, one head
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_steps_that_lead_nowhere(dtype):
+    # one row of a projection whose width is odd, caches of one sequence (or of one head) cut from buffers of odd widths
+    g = torch.Generator().manual_seed(4)
+    q = random(g, 2, 8 * 64 + 3, dtype=dtype).cuda()[:, :512].unflatten(1, (8, 64))[:1]
+    caches = [random(g, 2, 40 * 128 + 5, dtype=dtype).cuda()[:, :40 * 128].unflatten(1, (40, 2, 64))[:1] for _ in range(2)]
+    assert q.stride(0) % 2 == 1 and caches[0].stride(0) % 2 == 1
+    index = torch.tensor([[[1, 0], [2, -1]]], dtype=torch.int32, device="cuda")
+    at = torch.tensor(37, device="cuda")
+    out, lse = ba.block_attention(q, *caches, index, at, 8, 6, 0.125)
+    check_rows([0], [(0, 37)], q, *caches, index, out, lse, 8, 6, 0.125)
+    one = [torch.as_strided(c, (1, 40, 1, 64), (c.stride(0), 128, 63, 1)) for c in caches]
+    out, lse = ba.block_attention(q, *one, index[:, :1], at, 8, 6, 0.125)
+    check_rows([0], [(0, 37)], q, *one, index[:, :1], out, lse, 8, 6, 0.125)
+    # and into them
+    k, v = (random(g, 2, 2 * 64 + 1, dtype=dtype).cuda()[:, :128].unflatten(1, (2, 64))[:1] for _ in range(2))
+    f, plainly = ba.rotary_frequencies(64, device="cuda")[0], [c.clone(memory_format=torch.contiguous_format) for c in caches]
+    turned = ba.rotary_append(q, k, v, *caches, f, at)
+    assert torch.equal(turned, ba.rotary_append(q.contiguous(), k.contiguous(), v.contiguous(), *plainly, f, at))
+    assert all(torch.equal(a, b) for a, b in zip(caches, plainly))
+    within(turned, *plain.turned(q.cpu(), 37, f.cpu(), False, 1.0))
+    status_clear()
