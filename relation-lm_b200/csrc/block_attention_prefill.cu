@@ -10,7 +10,8 @@
 //   3. block_attention_window_kernel: per 64 consecutive (row, query head) entries the attention over the local windows,
 //      whose keys they share, joined with the pairs' partial results.
 //
-// An entry's arithmetic does not depend on its place in a tile, nor on the order of the sort: results are reproducible.
+// An entry's arithmetic depends neither on its place in a tile nor on the entries beside it, nor thereby on the order of the
+// sort: results are reproducible, those beside values that are not finite among them.
 // The workspace is reused from segment to segment, which also keeps most of it in L2.
 //
 // The tiles of head widths 64 and 128 and blocks of up to 64 keys multiply on tcgen05; other widths and blocks, and the windows,
@@ -233,12 +234,12 @@ template <int D> struct Running {
     }
 };
 
-// kKeys staged keys and values against a warp's 16 entries; an entry sees the keys [low, high) of them.  `careful`: some
-// value is not finite and not every entry sees every key, so a weight of zero must not meet it: the weighted sum is made
-// on the CUDA cores, of the keys that an entry sees.
+// kKeys staged keys and values against a warp's 16 entries; an entry sees the keys [low, high) of them.  `careful`, of this
+// lane's entries: some value is not finite and the entry may not see it, so a weight of zero must not meet it: the weighted
+// sum is made on the CUDA cores, of the keys that the entry sees.  In windows (kAscending) all entries of a warp are or none.
 template <typename T, int D, int kKeys, bool kAscending>
 __device__ __forceinline__ void take_keys(Running<D>& run, const uint32_t (&q)[D / 16][4], uint32_t keys, uint32_t values,
-                                          const int (&low)[2], const int (&high)[2], float scale_log2, bool careful,
+                                          const int (&low)[2], const int (&high)[2], float scale_log2, const bool (&careful)[2],
                                           const unsigned char* value_rows) {
     using S = TileShape<D>;
     const int lane = threadIdx.x & 31;
@@ -247,6 +248,7 @@ __device__ __forceinline__ void take_keys(Running<D>& run, const uint32_t (&q)[D
     // the warp's entries ascend: the first sees the first keys, the last the last ones.  16 keys that none sees are passed by
     const int first_seen = kAscending ? __shfl_sync(0xffffffffu, low[0], 0) : 0;
     const int last_seen = kAscending ? __shfl_sync(0xffffffffu, high[1], 31) : kKeys;
+    const bool any_careful = __any_sync(0xffffffffu, careful[0] || careful[1]);
     float s[kKeys / 8][4];
 #pragma unroll
     for (int n = 0; n < kKeys / 8; ++n)
@@ -306,7 +308,23 @@ __device__ __forceinline__ void take_keys(Running<D>& run, const uint32_t (&q)[D
             w[2 * j] = pack2<T>(x[0], x[1]);
             w[2 * j + 1] = pack2<T>(x[2], x[3]);
         }
-        if (careful) {
+        if (any_careful) {
+            if constexpr (!kAscending) {           // the other entries as ever: their sums do not hang on their neighbours
+#pragma unroll
+                for (int d = 0; d < D / 16; ++d) {
+                    uint32_t b[4];
+                    ldmatrix4_trans(b, values + (16 * n + value_row) * S::kRowBytes + 32 * d + 16 * value_half);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        float* acc = run.acc[2 * d + j];
+                        float sum[4] = {acc[0], acc[1], acc[2], acc[3]};
+                        mma16816<T>(sum, w, b[2 * j], b[2 * j + 1]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (!careful[i >> 1]) acc[i] = sum[i];
+                    }
+                }
+            }
 #pragma unroll 1
             for (int k = 0; k < 16; ++k) {
                 const int owner = (lane & ~3) | ((k & 7) >> 1), key = 16 * n + k;
@@ -314,7 +332,7 @@ __device__ __forceinline__ void take_keys(Running<D>& run, const uint32_t (&q)[D
                                           __shfl_sync(0xffffffffu, k < 8 ? w[1] : w[3], owner)};
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    if (key < low[i] || key >= high[i]) continue;
+                    if (!careful[i] || key < low[i] || key >= high[i]) continue;
                     const float2 pair = unpack2<T>(both[i]);
                     const float weight = (k & 1) ? pair.y : pair.x;
 #pragma unroll
@@ -433,7 +451,8 @@ __global__ void __launch_bounds__(kBpThreads) block_attention_tiles_kernel(const
             }
             const int left = cached - o;
             const int low[2] = {0, 0}, high[2] = {min(before[0] - o, left), min(before[1] - o, left)};
-            take_keys<T, D, kKeys, false>(run, q, keys, values, low, high, a.scale_log2, clipped && !finite, staged_values);
+            const bool careful[2] = {before[0] < cached && !finite, before[1] < cached && !finite};
+            take_keys<T, D, kKeys, false>(run, q, keys, values, low, high, a.scale_log2, careful, staged_values);
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -555,7 +574,8 @@ __global__ void __launch_bounds__(kTtRows, D == 64 ? 6 : 3) block_attention_tens
         }
         cp_async_commit();
         const int2 mine = entries[first + tid];
-        const int before = mine.x < 0 ? cached : min(max(g.t0 + (mine.x >> kBpRankBits) - a.window + 1, 0) - at, cached);
+        auto seen = [&](int pair) { return pair < 0 ? cached : min(max(g.t0 + (pair >> kBpRankBits) - a.window + 1, 0) - at, cached); };
+        const int before = seen(mine.x);
         cp_async_wait_all();
         fence_proxy_async();
         const bool clipped = __syncthreads_or(before < cached);
@@ -615,7 +635,8 @@ __global__ void __launch_bounds__(kTtRows, D == 64 ? 6 : 3) block_attention_tens
         const float base = top == kNegInf ? 0.0f : top;
         float2 sum2 = make_float2(0.0f, 0.0f);
         const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), base2 = make_float2(-base, -base);
-        const bool careful = clipped && !finite;
+        // an entry's own matter, so that its sums do not hang on its neighbours
+        auto careful = [&](int pair) { return !finite && seen(pair) < cached; };
 #pragma unroll
         for (int c = 0; c < kKeys / 16; ++c) {
             float x[16];
@@ -641,7 +662,7 @@ __global__ void __launch_bounds__(kTtRows, D == 64 ? 6 : 3) block_attention_tens
             const int row = mine.x >> kBpRankBits, rank = mine.x & ((1 << kBpRankBits) - 1);
             const int64_t entry = ((static_cast<int64_t>(row) * a.kv_heads + kv) * a.top + rank) * a.group + mine.y;
             reinterpret_cast<float2*>(g.base + p.plan.stats)[entry] = make_float2(top, sum2.x + sum2.y);
-            if (careful) {
+            if (careful(mine.x)) {
                 // the weighted sum on the CUDA cores, of the keys that the entry sees, 16 components at a time
                 float* sums = reinterpret_cast<float*>(g.base + p.plan.sums) + entry * D;
 #pragma unroll 1
@@ -670,45 +691,43 @@ __global__ void __launch_bounds__(kTtRows, D == 64 ? 6 : 3) block_attention_tens
                 }
             }
         }
-        if (!careful) {
-            fence_proxy_async();
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncthreads();
-            if (failed) break;
-            if (warp == 0) {
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const bool elected = elect_lane();
-#pragma unroll
-                for (int k = 0; k < kKeys / 16; ++k)
-                    umma_f16_if(tmem, smem_desc_sw128(queries_at) + 2 * k, value_desc(values_at + 2048 * k, S::kKeyBlock), kSums, k > 0, elected);
-                umma_commit_if(bar, elected);
-            }
-            if (!mbar_wait(bar, phase)) failed = 1;
-            phase ^= 1;
+        fence_proxy_async();
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncthreads();
+        if (failed) break;
+        if (warp == 0) {
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const bool elected = elect_lane();
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                float* to[2];
+            for (int k = 0; k < kKeys / 16; ++k)
+                umma_f16_if(tmem, smem_desc_sw128(queries_at) + 2 * k, value_desc(values_at + 2048 * k, S::kKeyBlock), kSums, k > 0, elected);
+            umma_commit_if(bar, elected);
+        }
+        if (!mbar_wait(bar, phase)) failed = 1;
+        phase ^= 1;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int2 other = entries[first + 32 * warp + 16 * half + (lane >> 2) + 8 * i];
-                    const int row = other.x >> kBpRankBits, rank = other.x & ((1 << kBpRankBits) - 1);
-                    const int64_t entry = ((static_cast<int64_t>(row) * a.kv_heads + kv) * a.top + rank) * a.group + other.y;
-                    to[i] = other.x < 0 ? nullptr : reinterpret_cast<float*>(g.base + p.plan.sums) + entry * D + 4 * (lane & 3);
-                }
+        for (int half = 0; half < 2; ++half) {
+            float* to[2];
 #pragma unroll
-                for (int b = 0; b < D / 64; ++b) {
-                    uint32_t v[32];
-                    tmem_ld_16x256b(tmem + (static_cast<uint32_t>(32 * warp + 16 * half) << 16) + 64 * b, v);
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            for (int i = 0; i < 2; ++i) {
+                const int2 other = entries[first + 32 * warp + 16 * half + (lane >> 2) + 8 * i];
+                const int row = other.x >> kBpRankBits, rank = other.x & ((1 << kBpRankBits) - 1);
+                const int64_t entry = ((static_cast<int64_t>(row) * a.kv_heads + kv) * a.top + rank) * a.group + other.y;
+                to[i] = other.x < 0 || careful(other.x) ? nullptr : reinterpret_cast<float*>(g.base + p.plan.sums) + entry * D + 4 * (lane & 3);
+            }
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
-                        if (to[i])
+            for (int b = 0; b < D / 64; ++b) {
+                uint32_t v[32];
+                tmem_ld_16x256b(tmem + (static_cast<uint32_t>(32 * warp + 16 * half) << 16) + 64 * b, v);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-                            for (int c = 0; c < 4; ++c)
-                                *reinterpret_cast<uint4*>(to[i] + 64 * b + 16 * c) =
-                                    make_uint4(v[8 * c + 2 * i], v[8 * c + 2 * i + 1], v[8 * c + 4 + 2 * i], v[8 * c + 4 + 2 * i + 1]);
-                }
+                for (int i = 0; i < 2; ++i)
+                    if (to[i])
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+                            *reinterpret_cast<uint4*>(to[i] + 64 * b + 16 * c) =
+                                make_uint4(v[8 * c + 2 * i], v[8 * c + 2 * i + 1], v[8 * c + 4 + 2 * i], v[8 * c + 4 + 2 * i + 1]);
             }
         }
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -808,7 +827,8 @@ __global__ void __launch_bounds__(kBpThreads, D <= 64 ? 4 : 2) block_attention_w
             const unsigned char* staged_values = memory + kBpEntries * S::kRowBytes + stage * kStage + kKeys * S::kRowBytes;
             // keys that every row of the tile sees may hold anything
             const bool all = at >= g.t0 + last_q + 1 - a.window && at + kKeys <= g.t0 + first_q + 1;
-            const bool careful = !all && __syncthreads_or(staged_not_finite<T, D, kKeys>(staged_values, threadIdx.x, kBpThreads));
+            const bool not_finite = !all && __syncthreads_or(staged_not_finite<T, D, kKeys>(staged_values, threadIdx.x, kBpThreads));
+            const bool careful[2] = {not_finite, not_finite};
             if (round == 0) load_queries<D>(q, staged_q + 16 * warp * S::kRowBytes, a.flip);
             const int low[2] = {from[0] - at, from[1] - at}, high[2] = {to[0] - at, to[1] - at};
             // a warp none of whose rows sees these keys passes

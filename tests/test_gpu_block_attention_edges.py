@@ -145,3 +145,46 @@ def test_steps_that_lead_nowhere(dtype):
     assert all(torch.equal(a, b) for a, b in zip(caches, plainly))
     within(turned, *plain.turned(q.cpu(), 37, f.cpu(), False, 1.0))
     status_clear()
+
+
+# ---------------------------------------------------------------------------- values that are not finite, and neighbours
+
+
+@pytest.mark.parametrize("dtype", HALF_TYPES)
+@pytest.mark.parametrize("width,block_size", [(64, 16), (64, 64), (128, 32), (32, 16), (96, 64), (64, 100)])
+def test_a_row_does_not_hang_on_its_neighbours(dtype, width, block_size):
+    # every block ends in a value that is not finite.  Rows that see whole blocks stay as they are, to the last bit, whether or
+    # not rows whose window begins within the same block choose it as well; and every call gives the same
+    length, window, heads = 1500, 24, 4
+    g = torch.Generator().manual_seed(width + block_size)
+    q = random(g, length, heads, width, dtype=dtype).cuda()
+    k_cache, v_cache = (random(g, 1, length, 2, width, dtype=dtype).cuda() for _ in range(2))
+    v_cache[0, block_size - 1::block_size, :, 5] = math.inf
+    t = torch.arange(length)
+    start = (t - window + 1).clamp(min=0)
+    whole = start // block_size                          # blocks that end before the window
+    far = (torch.rand(length, generator=g) * whole).int()
+    plain_rows = (t % 2 == 0) & (whole > 0)
+    alone = torch.where(plain_rows, far, -1).int()
+    beside = torch.where((t % 2 == 1) & (start % block_size > 0), start // block_size, alone).int()
+    assert int((beside >= 0).sum()) > int((alone >= 0).sum()) + 400
+
+    def call(index):
+        return ba.block_attention_prefill(q, k_cache, v_cache, index[:, None].cuda(), length, block_size, window, 0.125)
+
+    out, lse = call(alone)
+    assert not bool(out[plain_rows.cuda()][..., 5].isfinite().any()) and bool(out[plain_rows.cuda()][..., 6:].isfinite().all())
+    with_others, lse_with = call(beside)
+    rest = torch.arange(width) != 5
+    assert torch.equal(out[plain_rows.cuda()][..., rest], with_others[plain_rows.cuda()][..., rest])
+    assert torch.equal(lse[plain_rows.cuda()], lse_with[plain_rows.cuda()])
+    for _ in range(3):
+        again, lse_again = call(beside)
+        assert torch.equal(again.view(torch.int16), with_others.view(torch.int16)) and torch.equal(lse_again, lse_with)
+    cpu = [x.cpu() for x in (q, k_cache, v_cache)]
+    for i in range(200, length, 61):                     # the other components, against the 64-bit form
+        finite = cpu[2].nan_to_num(posinf=0.0)
+        want, want_lse, bound, lse_bound = plain.attend(cpu[0][i], cpu[1][0], finite[0], beside[i].expand(2, 1), i, block_size, window, 0.125)
+        within(with_others[i][..., rest], want[..., rest], bound[..., rest], i)
+        within(lse_with[i], want_lse, lse_bound)
+    status_clear()
