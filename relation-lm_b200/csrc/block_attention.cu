@@ -301,8 +301,8 @@ __global__ void __launch_bounds__(kBaThreads) block_attention_rows_kernel(const 
                 s[n][i] = power2(__fmul_rn(s[n][i], a.scale_log2) - top[i >> 1]);
                 sum[i >> 1] += s[n][i];
             }
-            p[2 * n] = pack2<T>(s[n][0], s[n][1]);
-            p[2 * n + 1] = pack2<T>(s[n][2], s[n][3]);
+            p[2 * n] = pack_weights<T>(s[n][0], s[n][1]);
+            p[2 * n + 1] = pack_weights<T>(s[n][2], s[n][3]);
         }
         l[0] = l[0] * grow[0] + sum[0];
         l[1] = l[1] * grow[1] + sum[1];
@@ -340,6 +340,7 @@ __global__ void __launch_bounds__(kBaThreads) block_attention_rows_kernel(const 
     }
     __syncthreads();                                     // the sums of a warp may reach into another warp's ring
     float* parts = reinterpret_cast<float*>(memory);
+    constexpr float kDown = 1.0f / kWeightFactor<T>;
 #pragma unroll
     for (int n = 0; n < D / 8; ++n)
 #pragma unroll
@@ -347,7 +348,7 @@ __global__ void __launch_bounds__(kBaThreads) block_attention_rows_kernel(const 
             const int h = (lane >> 2) + 8 * i;
             if (h < n_heads)
                 *reinterpret_cast<float2*>(parts + (warp * 16 + h) * D + 8 * n + 2 * (lane & 3)) =
-                    make_float2(acc[n][2 * i], acc[n][2 * i + 1]);
+                    make_float2(acc[n][2 * i] * kDown, acc[n][2 * i + 1] * kDown);
         }
     join_and_write<T, D, kBaWarps, 16>(a, row, first_head, n_heads, rank, parts, part_m, part_l,
                                        reinterpret_cast<float*>(memory + P::kParts), joined_m, joined_l);

@@ -51,6 +51,15 @@ template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) 
     return *reinterpret_cast<uint32_t*>(&v);
 }
 
+// Softmax weights (powers of two of at most zero) as operands of the tensor cores are rounded to 16 bits: half a step, 2^-8 (bf16)
+// or 2^-11 (fp16) of each weight, beside the same rounding of the result; twice the bits would take twice the products.
+// In fp16 weights below 2^-14 would lose bits and those below 2^-25 vanish, however many or however large their values are,
+// so there they are carried 2^15-fold: all bits down to 2^-29 of the largest, some down to 2^-39.  The sums take the factor out again.
+template <typename T> constexpr float kWeightFactor = std::is_same<T, __half>::value ? 32768.0f : 1.0f;
+template <typename T> __device__ __forceinline__ uint32_t pack_weights(float a, float b) {
+    return pack2<T>(a * kWeightFactor<T>, b * kWeightFactor<T>);
+}
+
 template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t v);
 template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {
     return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));

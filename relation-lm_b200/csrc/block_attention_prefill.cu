@@ -5,8 +5,8 @@
 //
 //   1. block_attention_sort_kernel: per segment of up to 4096 rows a counting sort of its pairs by block, and the list of
 //      tiles: runs of up to 256 (row, query head) entries that share a block;
-//   2. block_attention_tiles_kernel: per tile softmax(q K') V of the entries with the block, unnormalised, with the
-//      maximum and the sum, to the pair's place in the workspace (fp32);
+//   2. block_attention_tiles_kernel: per tile softmax(q K') V of the entries with the block, unnormalised (and times the factor
+//      that fp16 weights carry), with the maximum and the sum, to the pair's place in the workspace (fp32);
 //   3. block_attention_window_kernel: per 64 consecutive (row, query head) entries the attention over the local windows,
 //      whose keys they share, joined with the pairs' partial results.
 //
@@ -305,8 +305,8 @@ __device__ __forceinline__ void take_keys(Running<D>& run, const uint32_t (&q)[D
                 x[i] = power2(__fmul_rn(x[i], scale_log2) - top[i >> 1]);
                 run.l[i >> 1] += x[i];
             }
-            w[2 * j] = pack2<T>(x[0], x[1]);
-            w[2 * j + 1] = pack2<T>(x[2], x[3]);
+            w[2 * j] = pack_weights<T>(x[0], x[1]);
+            w[2 * j + 1] = pack_weights<T>(x[2], x[3]);
         }
         if (any_careful) {
             if constexpr (!kAscending) {           // the other entries as ever: their sums do not hang on their neighbours
@@ -655,8 +655,8 @@ __global__ void __launch_bounds__(kTtRows, D == 64 ? 6 : 3) block_attention_tens
 #pragma unroll
             for (int h = 0; h < 2; ++h)
                 *reinterpret_cast<uint4*>(memory + swizzled(tid, 2 * c + h, S::kQueryBlock)) =
-                    make_uint4(pack2<T>(x[8 * h], x[8 * h + 1]), pack2<T>(x[8 * h + 2], x[8 * h + 3]),
-                               pack2<T>(x[8 * h + 4], x[8 * h + 5]), pack2<T>(x[8 * h + 6], x[8 * h + 7]));
+                    make_uint4(pack_weights<T>(x[8 * h], x[8 * h + 1]), pack_weights<T>(x[8 * h + 2], x[8 * h + 3]),
+                               pack_weights<T>(x[8 * h + 4], x[8 * h + 5]), pack_weights<T>(x[8 * h + 6], x[8 * h + 7]));
         }
         if (mine.x >= 0) {
             const int row = mine.x >> kBpRankBits, rank = mine.x & ((1 << kBpRankBits) - 1);
@@ -863,7 +863,7 @@ __global__ void __launch_bounds__(kBpThreads, D <= 64 ? 4 : 2) block_attention_w
         run.l[i] += __shfl_xor_sync(0xffffffffu, run.l[i], 2);
         if (first + 16 * warp + (lane >> 2) + 8 * i > last) continue;
         const int64_t to_row = (first_row + row_of[i]) * a.heads + kv * a.group + head_of[i];
-        const float scale = run.l[i] == 0.0f ? 0.0f : 1.0f / run.l[i];
+        const float scale = run.l[i] == 0.0f ? 0.0f : 1.0f / (run.l[i] * kWeightFactor<T>);
 #pragma unroll
         for (int c = 0; c < D / 8; ++c)
             *reinterpret_cast<uint32_t*>(a.out + (to_row * D + 8 * c + 2 * (lane & 3)) * 2) =

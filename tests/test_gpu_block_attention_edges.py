@@ -188,3 +188,45 @@ def test_a_row_does_not_hang_on_its_neighbours(dtype, width, block_size):
         within(with_others[i][..., rest], want[..., rest], bound[..., rest], i)
         within(lse_with[i], want_lse, lse_bound)
     status_clear()
+
+
+# ---------------------------------------------------------------------------- weights far below the largest
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("form", ("decode", "rows", "prefill"))
+@pytest.mark.parametrize("width,block_size", [(64, 64), (128, 32), (32, 16), (64, 100)])
+def test_many_small_weights_count(dtype, form, width, block_size):
+    # one key of every 50 outweighs each of the others 2^26-fold, but its value is zero and theirs are large: the result is
+    # theirs.  Scores are whole powers of two, so that nothing but the rounding of the weights and of the result is left
+    length, window, heads, top = 1300, 120, 4, 4          # whole sequences: as many rows as take the three passes
+    g = torch.Generator().manual_seed(width)
+    at = [(0, 897)] if form == "decode" else [(0, t) for t in range(700, 1300, 29)] if form == "rows" else plain.places(form, 1, 0, 0, length)
+    n = len(at)
+    q = torch.zeros(n, heads, width, dtype=dtype)
+    q[..., 0] = 1.0
+    k_cache = torch.zeros(1, length, 1, width, dtype=dtype)
+    k_cache[0, ::50, 0, 0] = 26.0
+    v_cache = (torch.rand(1, length, 1, width, generator=g) * 3.0e4 + 3.0e4).to(dtype)
+    v_cache[0, ::50] = 0.0
+    index = torch.randint(0, -(-length // block_size), (n, 1, top), generator=g, dtype=torch.int32)
+    scale = math.log(2.0)
+    call = {"decode": ba.block_attention, "rows": ba.block_attention_rows, "prefill": ba.block_attention_prefill}[form]
+    out, lse = call(q.cuda(), k_cache.cuda(), v_cache.cuda(), index.cuda(), *plain.where(form, at, length), block_size, window, scale)
+    step = plain.HALF_STEP[dtype]
+    for i in range(0, n, 1 + n // 60):
+        t = at[i][1]
+        start = max(0, t - window + 1)
+        keys = set(range(start, t + 1))
+        for b in index[i, 0].tolist():
+            keys |= set(range(b * block_size, min((b + 1) * block_size, start)))
+        keys = sorted(keys)
+        p = torch.exp2(k_cache[0, keys, 0, 0].double())
+        want = (p @ v_cache[0, keys, 0].double()) / p.sum()
+        # the scale times log2(e) in 32 bits: 2^-24 each and of the product, times 26 in the exponent and ln 2; powers (2 ulp),
+        # sums over the keys; weights and the result rounded to the type, the latter to fp16's smallest steps
+        weight = 2 * 3 * 2.0 ** -24 * 26 * math.log(2.0) + (len(keys) + 16) * 2.0 ** -24
+        bound = (weight + (2 * step if dtype != torch.float32 else step)) * 1.01 * want + (2.0 ** -25 if dtype == torch.float16 else 0.0)
+        within(out[i], want.expand(heads, width), bound.expand(heads, width), (i, t))
+        within(lse[i], p.sum().log().expand(heads), torch.full((heads,), 1e-5, dtype=torch.float64))
+    status_clear()
