@@ -773,7 +773,9 @@ int rlm_sequence_state(
  * sequence and position, a negative position marks a row of padding; else `position`: row i is sequence i, all at
  * *position (n_rows == n_seq); else n_rows == n_seq * query_length rows, row i at position i % query_length of sequence
  * i / query_length.  Rows outside the caches set RLM_DEV_POSITION.  Both they and rows of padding give zeros (route: index
- * -1, score -inf; attention: lse -inf) and write nothing into a cache.
+ * -1, score -inf; attention: lse -inf) and write nothing into a cache.  rlm_block_route knows no cache, only block
+ * statistics: beyond them all their blocks are complete, so only a sequence outside them, a negative *position and one
+ * above 2^31 - 2 are told.
  */
 
 /*
@@ -794,7 +796,8 @@ int rlm_rotary_append(const void* query, const void* key, const void* value, voi
  * The `top_blocks` (<= 128) best blocks of every row by the score of rlm_relation_select_packed's anchor stream, among
  * the blocks that are complete at the row's position and, with `strict_valid`, end before its local window: out_index,
  * out_score [n_rows, top_blocks] in descending order, ties to the lowest block, -1 and -inf where there are fewer.
- * Scores are compared in 64 bits.  A score that is NaN or -inf is no choice.
+ * Scores are compared in 64 bits.  A score that is NaN or -inf is no choice.  The selectors compare theirs in 32 bits, and
+ * take blocks above -1e30 only: where two scores are as near as 32 bits tell apart the choices may differ.
  */
 int rlm_block_route(const void* router_query, int64_t query_row_stride, const void* block_mean, const void* block_std,
                     const void* gamma, const void* bias, const int64_t* position, const int32_t* row_batch,

@@ -12,7 +12,8 @@ Each comes in the forms of the selectors: for one decode position (``position``,
 sequence), for rows with a sequence and a position of their own (``*_rows``; int32 ``row_batch`` and ``row_position``, a
 negative position marks a row of padding) and for whole sequences (``*_prefill``; row ``b * query_length + t``).  Rows of
 padding and rows outside the caches give zeros (index -1, score and lse -inf) and write nothing; the latter also set the
-status word.  Nothing here has a derivative.
+status word.  ``route_blocks`` knows no cache: only sequences outside its statistics count there, and a position beyond them
+has all their blocks behind it.  Nothing here has a derivative.
 """
 from __future__ import annotations
 
@@ -116,7 +117,8 @@ def route_blocks(router_query: Tensor, block_mean: Tensor, block_std: Tensor, ga
     ``router_query [N, 64]``, statistics ``[B, blocks, 4, 16]``, ``gamma [4]``, ``bias [4, buckets]``.  Blocks that are complete
     at the row's position take part, with ``strict_valid`` only those that end before its local window.  Ties go to the
     lowest block; places without a block hold -1 and -inf.  Scores are compared in 64 bits, so the choice does not depend
-    on the form of the call.
+    on the form of the call.  (``relation_select_packed`` compares the same scores in 32 bits and takes those above -1e30
+    only: where two are as near as 32 bits tell apart, it may look into another block.)
     """
     return _route_blocks(router_query, block_mean, block_std, gamma, bias, position, block_size, local_window, top_blocks,
                          strict_valid)

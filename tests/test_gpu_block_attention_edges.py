@@ -230,3 +230,90 @@ def test_many_small_weights_count(dtype, form, width, block_size):
         within(out[i], want.expand(heads, width), bound.expand(heads, width), (i, t))
         within(lse[i], p.sum().log().expand(heads), torch.full((heads,), 1e-5, dtype=torch.float64))
     status_clear()
+
+
+# ---------------------------------------------------------------------------- the choice, and the selectors beside it
+
+
+def _statistics(g, batch, blocks, dtype=torch.float32):
+    mean, std = random(g, batch, blocks, 4, 16, dtype=dtype, scale=0.5), random(g, batch, blocks, 4, 16, dtype=dtype, scale=0.5).abs()
+    return mean, std, random(g, 4), random(g, 4, 9)
+
+
+@pytest.mark.parametrize("place", [(2, 5), (-1, 5), (2, 0), (1 << 30, 1 << 30)])
+def test_route_tells_each_row_outside_the_statistics(place):
+    from relation_lm.kernels import _abi
+
+    x = [v.cuda() for v in _statistics(torch.Generator().manual_seed(1), 2, 6)]
+    q = torch.randn(1, 64, device="cuda")
+    row = [torch.tensor([v], dtype=torch.int32, device="cuda") for v in place]
+    index, score = ba.route_blocks_rows(q, *x, *row, 4, 2, 3, True)
+    assert _abi.read_status() == 2 and index.tolist() == [[-1] * 3] and score.tolist() == [[-math.inf] * 3]
+    index, score = ba.route_blocks(q.expand(2, 64).contiguous(), *x, torch.tensor(-1, device="cuda"), 4, 2, 3, True)
+    assert _abi.read_status() == 2 and index.tolist() == [[-1] * 3] * 2
+
+
+@pytest.mark.parametrize("blocks,block_size,top", [(2, 4, 1), (6, 4, 3), (700, 16, 40)])
+@pytest.mark.parametrize("beyond", (0, 1, 1000, 0x7fffffff - 700 * 16 - 1))
+def test_beyond_the_statistics_all_blocks_are_complete(blocks, block_size, top, beyond):
+    g = torch.Generator().manual_seed(blocks)
+    mean, std, gamma, bias = _statistics(g, 2, blocks)
+    q, t = random(g, 2, 64), blocks * block_size + beyond
+    given = [v.cuda() for v in (q, mean, std, gamma, bias)]
+    at = torch.tensor([t, t], dtype=torch.int32, device="cuda")
+    index, score = ba.route_blocks_rows(*given, torch.arange(2, dtype=torch.int32, device="cuda"), at, block_size, 2, top, False)
+    same, same_score = ba.route_blocks(*given, torch.tensor(t, device="cuda"), block_size, 2, top, False)
+    for b in range(2):
+        want, value = plain.route(q[b], mean[b], std[b], gamma, bias, t, block_size, 2, top, False)
+        assert index[b].tolist() == want == same[b].tolist()
+        value = torch.tensor(value, dtype=torch.float64)
+        within(score[b], value, 2.0 ** -24 * value.abs() + 1e-12)
+    assert torch.equal(score, same_score)
+    status_clear()
+
+
+@pytest.mark.parametrize("strict", (False, True))
+@pytest.mark.parametrize("window", (1, 40))
+def test_route_chooses_by_the_scores_of_the_selectors(strict, window):
+    import oracle
+
+    batch, blocks, block_size, top = 3, 64, 16, 7
+    g = torch.Generator().manual_seed(window)
+    mean, std, gamma, bias = _statistics(g, batch, blocks)
+    length = blocks * block_size
+    q = random(g, batch * length, 64)
+    index, score = (x.cpu() for x in ba.route_blocks_prefill(*[v.cuda() for v in (q, mean, std, gamma, bias)], length, block_size,
+                                                             window, top, strict))
+    for i in range(0, batch * length, 37):
+        b, t = divmod(i, length)
+        ours = oracle.block_scores(mean[b], std[b], q[i], gamma, bias, t, length, window, strict).double()
+        # a head's score in 32 bits: 20 operations on the sum of its magnitudes, logarithms and exponentials to 2^-20
+        size = (q[i].abs().view(4, 16) * mean[b].abs()).sum(-1) + torch.nn.functional.softplus(gamma) * (q[i].abs().view(4, 16) * std[b]).sum(-1)
+        error = float((20 * 2.0 ** -24 * (size / 4 + bias.abs().amax())).max()) + 2.0 ** -19
+        some = index[i] >= 0
+        assert int(some.sum()) == min(top, int((ours > -math.inf).sum()))
+        chosen = ours[index[i][some].long()]
+        assert bool(((score[i][some].double() - chosen).abs() <= error).all())
+        rest = ours.clone()
+        rest[index[i][some].long()] = -math.inf
+        assert bool((chosen >= rest.max() - 2 * error).all()) and bool((chosen[1:] <= chosen[:-1] + 2 * error).all())
+
+
+@pytest.mark.parametrize("top", (1, 4))
+def test_route_chooses_the_blocks_that_the_selector_looks_into(top):
+    # every remote key scores the same and more than the window's one: the anchor is the first row of the first chosen block
+    from relation_lm.kernels.relation_select import relation_select_packed
+
+    batch, blocks, block_size, t = 8, 32, 16, 509
+    g = torch.Generator().manual_seed(top)
+    mean, std, gamma, bias = (v.cuda() for v in _statistics(g, batch, blocks))
+    rq, query = random(g, batch, 64).cuda(), torch.ones(batch, 64, device="cuda")
+    keys = torch.ones(batch, blocks * block_size, 64, device="cuda")
+    keys[:, t] = -1.0
+    partner = torch.zeros(batch, blocks * block_size, 128, device="cuda")
+    position = torch.tensor(t, device="cuda")
+    anchor = relation_select_packed(query, keys, rq, mean, std, gamma, bias, partner[:, 0].contiguous(), partner, keys, mean, std, gamma,
+                                    bias, position, 1, top, 8, True)[0]
+    index, _ = ba.route_blocks(rq, mean, std, gamma, bias, position, block_size, 1, top, True)
+    assert torch.equal(anchor, index.amin(1) * block_size) and len(set(index.flatten().tolist())) > 4
+    status_clear()
