@@ -317,3 +317,44 @@ def test_route_chooses_the_blocks_that_the_selector_looks_into(top):
     index, _ = ba.route_blocks(rq, mean, std, gamma, bias, position, block_size, 1, top, True)
     assert torch.equal(anchor, index.amin(1) * block_size) and len(set(index.flatten().tolist())) > 4
     status_clear()
+
+
+# ---------------------------------------------------------------------------- several rows a CTA
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("form", ("rows", "prefill"))
+@pytest.mark.parametrize("batch,length,heads,kv_heads,width,rotary,interleaved", [
+    (3, 397, 8, 2, 64, 64, False), (1, 1184, 16, 4, 128, 64, True), (5, 1001, 2, 1, 64, 64, False), (2, 2999, 3, 3, 32, 16, True),
+    (7, 2801, 1, 1, 8, 8, False), (3, 6667, 1, 1, 16, 0, False), (2, 3001, 1, 1, 7, 4, True), (1, 5003, 1, 1, 1024, 1024, False)])
+def test_rotary_append_of_many_rows(dtype, form, batch, length, heads, kv_heads, width, rotary, interleaved):
+    # as many rows as put several into a CTA, the last of which is short: bit for bit what a few rows at a time give
+    g = torch.Generator().manual_seed(length)
+    n = batch * length
+    q, k, v = (random(g, n, h, width, dtype=dtype).cuda() for h in (heads, kv_heads, kv_heads))
+    before = [random(g, batch, length + 3, kv_heads, width, dtype=dtype).cuda() for _ in range(2)]
+    f, magnitude = ba.rotary_frequencies(rotary, scaling="by_parts", factor=2.0, trained_context=64)
+    f = f.cuda()
+    order = torch.randperm(n, generator=g) if form == "rows" else torch.arange(n)
+    row_batch, row_position = (order // length).int(), (order % length).int()
+    if form == "rows":
+        row_position[order % 11 == 3] = -1               # rows of padding
+    caches, few = [c.clone() for c in before], [c.clone() for c in before]
+    rows = row_batch.cuda(), row_position.cuda()
+    if form == "rows":
+        out = ba.rotary_append_rows(q, k, v, *caches, f, *rows, interleaved, magnitude)
+    else:
+        out = ba.rotary_append_prefill(q, k, v, *caches, f, length, interleaved, magnitude)
+    parts = [slice(i, min(i + 500, n)) for i in range(0, n, 500)]
+    want = torch.cat([ba.rotary_append_rows(q[s], k[s], v[s], *few, f, *(r[s] for r in rows), interleaved, magnitude) for s in parts])
+    assert torch.equal(out, want) and all(torch.equal(a, b) for a, b in zip(caches, few))
+    for i in [0, 1, n - 1] + torch.randint(0, n, (20,), generator=g).tolist():
+        b, t = int(row_batch[i]), int(row_position[i])
+        if t < 0:
+            assert not out[i].any()
+            continue
+        within(out[i], *plain.turned(q[i].cpu(), t, f.cpu(), interleaved, magnitude))
+        within(caches[0][b, t], *plain.turned(k[i].cpu(), t, f.cpu(), interleaved, magnitude))
+        assert torch.equal(caches[1][b, t], v[i])
+    assert all(torch.equal(c[:, length:], o[:, length:]) for c, o in zip(caches, before))
+    status_clear()
