@@ -358,3 +358,184 @@ def test_rotary_append_of_many_rows(dtype, form, batch, length, heads, kv_heads,
         assert torch.equal(caches[1][b, t], v[i])
     assert all(torch.equal(c[:, length:], o[:, length:]) for c, o in zip(caches, before))
     status_clear()
+
+
+# ---------------------------------------------------------------------------- the three passes of whole sequences
+
+
+def passes_of(q, k_cache, index, length, block_size, window):
+    """The workspace of a whole-sequence call, in bytes: above zero where it takes the three passes, and of several launches
+    where it is less than the partial results of all rows."""
+    import ctypes
+
+    from relation_lm.kernels import _abi
+
+    size = ctypes.c_int64(-1)
+    index = index if index.dim() == 3 else index[:, None].expand(-1, k_cache.size(2), -1)
+    steps = (ctypes.c_int64 * 10)(*q.stride()[:2], *k_cache.stride()[:3], *k_cache.stride()[:3], *index.stride()[:2])
+    assert _abi.LIB.rlm_block_attention_workspace(steps, q.size(0), k_cache.size(0), k_cache.size(1), length, q.size(1), k_cache.size(2),
+                                                  q.size(2), index.size(2), block_size, window, _abi.code(q), ctypes.byref(size)) == 0
+    return size.value
+
+
+def _whole(seed, dtype, batch, length, heads, kv_heads, width, block_size, top):
+    g = torch.Generator().manual_seed(seed)
+    n = batch * length
+    q = random(g, n, heads, width, dtype=dtype).cuda()
+    caches = [random(g, batch, length, kv_heads, width, dtype=dtype).cuda() for _ in range(2)]
+    t = torch.arange(length).repeat(batch)
+    index = (torch.rand(n, kv_heads, top, generator=g) * (t[:, None, None] // block_size + 2)).int() - 1
+    return q, *caches, index.cuda()
+
+
+def _check_whole(x, length, block_size, window, scale, out, lse, every):
+    q, k_cache, v_cache, index = (v.cpu() for v in x)
+    at = [divmod(i, length) for i in range(q.size(0))]
+    check_rows(range(0, q.size(0), every), at, q, k_cache, v_cache, index, out, lse, block_size, window, scale)
+
+
+CASES = [(torch.bfloat16, 2, 601, 8, 2, 64, 64, 40, 3), (torch.float16, 1, 1100, 4, 2, 96, 32, 17, 5), (torch.float16, 2, 700, 8, 2, 128, 16, 0, 20)]
+
+
+@pytest.mark.parametrize("case", CASES)
+def test_three_passes_on_two_streams_at_once(case):
+    dtype, batch, length, heads, kv_heads, width, block_size, window, top = case
+    xs = [_whole(seed, dtype, batch, length, heads, kv_heads, width, block_size, top) for seed in range(2)]
+    rest = (length, block_size, window, 0.125)
+    assert all(passes_of(x[0], x[1], x[3], length, block_size, window) > 0 for x in xs)
+    want = [ba.block_attention_prefill(*x, *rest) for x in xs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in xs], [[], []]
+    for _ in range(12):
+        for x, s, keep in zip(xs, streams, got):
+            with torch.cuda.stream(s):
+                keep.append(ba.block_attention_prefill(*x, *rest))
+    torch.cuda.synchronize()
+    for x, w, keep in zip(xs, want, got):
+        _check_whole(x, *rest, *w, 97)
+        assert all(torch.equal(a, b) for r in keep for a, b in zip(r, w))
+    status_clear()
+
+
+@pytest.mark.parametrize("case", CASES)
+def test_three_passes_by_programmatic_launch(case):
+    from relation_lm.kernels import _abi
+
+    dtype, batch, length, heads, kv_heads, width, block_size, window, top = case
+    x = _whole(3, dtype, batch, length, heads, kv_heads, width, block_size, top)
+    assert passes_of(x[0], x[1], x[3], length, block_size, window) > 0
+    f = ba.rotary_frequencies(width, device="cuda")[0]
+
+    def layer():
+        caches = [torch.zeros_like(c) for c in x[1:3]]
+        q = ba.rotary_append_prefill(x[0], x[1].flatten(0, 1), x[2].flatten(0, 1), *caches, f, length)
+        first = ba.block_attention_prefill(q, *caches, x[3], length, block_size, window, 0.125)
+        return (q, *caches, *first, *ba.block_attention_prefill(first[0], *caches, x[3], length, block_size, window, 0.125))
+
+    want, chained = layer(), _abi.programmatic_launch(layer)
+    for _ in range(6):
+        assert all(torch.equal(a, b) for a, b in zip(want, chained()))
+    _check_whole((want[0], want[1], want[2], x[3]), length, block_size, window, 0.125, want[3], want[4], 97)
+    status_clear()
+
+
+@pytest.mark.parametrize("programmatic", (False, True))
+def test_several_launches_over_one_workspace(programmatic):
+    # more segments than fit the workspace: it is used again and again, also while the launch before it is still at its end
+    from relation_lm.kernels import _abi
+
+    batch, length, heads, kv_heads, width, block_size, window, top = 24, 1024, 16, 2, 128, 64, 33, 8
+    x = _whole(5, torch.bfloat16, batch, length, heads, kv_heads, width, block_size, top)
+    size = passes_of(x[0], x[1], x[3], length, block_size, window)
+    assert 0 < size < batch * length * heads * top * width * 4 / 2
+    call = _abi.programmatic_launch(ba.block_attention_prefill) if programmatic else ba.block_attention_prefill
+    out, lse = call(*x, length, block_size, window, 0.0884)
+    again, lse_again = call(*x, length, block_size, window, 0.0884)
+    assert torch.equal(out, again) and torch.equal(lse, lse_again)
+    for b in range(batch):                               # a sequence alone fits the workspace
+        rows = slice(b * length, (b + 1) * length)
+        alone, lse_alone = ba.block_attention_prefill(x[0][rows], x[1][b:b + 1], x[2][b:b + 1], x[3][rows], length, block_size, window, 0.0884)
+        assert torch.equal(out[rows], alone) and torch.equal(lse[rows], lse_alone), b
+    _check_whole(x, length, block_size, window, 0.0884, out, lse, 1777)
+    status_clear()
+
+
+@pytest.mark.parametrize("case", CASES)
+def test_three_passes_in_captured_graphs(case):
+    # two graphs of one memory pool, replayed in turn and with new inputs, and two graphs of their own at once
+    dtype, batch, length, heads, kv_heads, width, block_size, window, top = case
+    rest = (length, block_size, window, 0.125)
+    xs = [_whole(seed, dtype, batch, length, heads, kv_heads, width, block_size, top) for seed in (7, 8)]
+    fresh = [_whole(seed, dtype, batch, length, heads, kv_heads, width, block_size, top) for seed in (9, 10)]
+    want, want_fresh = ([ba.block_attention_prefill(*x, *rest) for x in many] for many in (xs, fresh))
+    assert passes_of(xs[0][0], xs[0][1], xs[0][3], length, block_size, window) > 0
+    torch.cuda.synchronize()
+
+    def capture(x, pool=None):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            out = ba.block_attention_prefill(*x, *rest)
+        return graph, out
+
+    first, out = capture(xs[0])
+    second, out2 = capture(xs[1], first.pool())
+    apart, out3 = capture(xs[1])
+    for _ in range(3):
+        for graph in (first, second):
+            graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for r, w in zip((out, out2), want) for a, b in zip(r, w))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(6):
+        for graph, s in zip((first, apart), streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for r, w in zip((out, out3), want) for a, b in zip(r, w))
+    for x, y in zip(xs, fresh):
+        for a, b in zip(x, y):
+            a.copy_(b)
+    first.replay()
+    second.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for r, w in zip((out, out2), want_fresh) for a, b in zip(r, w))
+    status_clear()
+
+
+@pytest.mark.parametrize("dtype", HALF_TYPES)
+def test_whole_sequence_layer_by_the_three_passes(dtype):
+    """rotary_append -> router_cache_update -> route_blocks -> block_attention over whole sequences that are long enough for
+    the passes, and the last positions of the same layer one by one."""
+    from relation_lm.kernels.router_cache import router_cache_update
+
+    batch, length, block, heads, kv_heads, width, window, top = 2, 800, 16, 4, 2, 64, 30, 3
+    g = torch.Generator().manual_seed(12)
+    n = batch * length
+    q, k, v = (random(g, n, h, width, dtype=dtype).cuda() for h in (heads, kv_heads, kv_heads))
+    rq, rk = random(g, n, 64, dtype=dtype).cuda(), random(g, batch, length, 64, dtype=dtype).cuda()
+    conv, gamma, bias = random(g, 64, 3, scale=0.1).cuda(), random(g, 4).cuda(), random(g, 4, 8).cuda()
+    f, magnitude = ba.rotary_frequencies(width, scaling="by_parts", factor=2.0, trained_context=400, device="cuda")
+    caches = [torch.zeros(batch, length, kv_heads, width, device="cuda", dtype=dtype) for _ in range(2)]
+    turned = ba.rotary_append_prefill(q, k, v, *caches, f, length, True, magnitude)
+    router = ([torch.zeros(batch, length, 64, device="cuda", dtype=dtype) for _ in range(4)]
+              + [torch.zeros(batch, length // block, 4, 16, device="cuda", dtype=dtype) for _ in range(4)])
+    for t in range(length):
+        router_cache_update(rk[:, t].contiguous(), rk[:, t].contiguous(), *router, conv, conv, torch.tensor(t, device="cuda"), block)
+    index, score = ba.route_blocks_prefill(rq, router[4], router[5], gamma, bias, length, block, window, top, True)
+    assert passes_of(turned, caches[0], index, length, block, window) > 0
+    out, lse = ba.block_attention_prefill(turned, *caches, index, length, block, window, 0.125)
+    for t in (length - 1, length - 17, 401, 30, 0):
+        rows = torch.arange(batch, device="cuda") * length + t
+        at = torch.tensor(t, device="cuda")
+        step = ba.rotary_append(q[rows], k[rows], v[rows], *[torch.zeros_like(c) for c in caches], f, at, True, magnitude)
+        assert torch.equal(step, turned[rows])
+        one, one_score = ba.route_blocks(rq[rows], router[4], router[5], gamma, bias, at, block, window, top, True)
+        assert torch.equal(one, index[rows]) and torch.equal(one_score, score[rows])
+        step_out, step_lse = ba.block_attention(step, *caches, one, at, block, window, 0.125)
+        for b in range(batch):
+            want, want_lse, bound, lse_bound = plain.attend(step[b].cpu(), caches[0][b].cpu(), caches[1][b].cpu(), one[b].cpu().expand(2, -1), t,
+                                                            block, window, 0.125)
+            for y, z in ((step_out[b], step_lse[b]), (out[rows[b]], lse[rows[b]])):
+                within(y, want, bound, t)
+                within(z, want_lse, lse_bound, t)
+    status_clear()
