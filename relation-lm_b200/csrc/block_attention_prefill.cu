@@ -923,11 +923,13 @@ int launch_tiles(const PrefillArgs& p, int segments, void* stream) {
             return check_launch("block_attention_tensor_tiles_kernel");
         }
     }
-    constexpr int smem = (2 * kBpEntries + 2 * kKeys) * TileShape<D>::kRowBytes;
-    if (smem > 48 * 1024)
-        if (int rc = allow_large_smem(reinterpret_cast<const void*>(&block_attention_tiles_kernel<T, D, kKeys>), kSmemDynamicLimit)) return rc;
-    launch_kernel(block_attention_tiles_kernel<T, D, kKeys>, grid, dim3(kBpThreads), smem, stream, p);
-    count_launch();
+    if constexpr (D % 64 != 0 || kKeys == 64) {    // widths 64 and 128: only blocks of more keys than that come here
+        constexpr int smem = (2 * kBpEntries + 2 * kKeys) * TileShape<D>::kRowBytes;
+        if (smem > 48 * 1024)
+            if (int rc = allow_large_smem(reinterpret_cast<const void*>(&block_attention_tiles_kernel<T, D, kKeys>), kSmemDynamicLimit)) return rc;
+        launch_kernel(block_attention_tiles_kernel<T, D, kKeys>, grid, dim3(kBpThreads), smem, stream, p);
+        count_launch();
+    }
     return check_launch("block_attention_tiles_kernel");
 }
 
