@@ -234,12 +234,12 @@ template <int D> struct Running {
     }
 };
 
-// kKeys staged keys and values against a warp's 16 entries; an entry sees the keys [low, high) of them.  `careful`, of this
-// lane's entries: some value is not finite and the entry may not see it, so a weight of zero must not meet it: the weighted
-// sum is made on the CUDA cores, of the keys that the entry sees.  In windows (kAscending) all entries of a warp are or none.
+// kKeys staged keys and values against a warp's 16 entries; an entry sees the keys [low, high) of them.  `careful`: some value
+// is not finite and not every entry sees every key, so a weight of zero must not meet it: the weighted sums of this lane's
+// entries that are `cut` are made on the CUDA cores, of the keys that they see.  In windows (kAscending) all entries are cut.
 template <typename T, int D, int kKeys, bool kAscending>
 __device__ __forceinline__ void take_keys(Running<D>& run, const uint32_t (&q)[D / 16][4], uint32_t keys, uint32_t values,
-                                          const int (&low)[2], const int (&high)[2], float scale_log2, const bool (&careful)[2],
+                                          const int (&low)[2], const int (&high)[2], float scale_log2, bool careful, const bool (&cut)[2],
                                           const unsigned char* value_rows) {
     using S = TileShape<D>;
     const int lane = threadIdx.x & 31;
@@ -248,7 +248,6 @@ __device__ __forceinline__ void take_keys(Running<D>& run, const uint32_t (&q)[D
     // the warp's entries ascend: the first sees the first keys, the last the last ones.  16 keys that none sees are passed by
     const int first_seen = kAscending ? __shfl_sync(0xffffffffu, low[0], 0) : 0;
     const int last_seen = kAscending ? __shfl_sync(0xffffffffu, high[1], 31) : kKeys;
-    const bool any_careful = __any_sync(0xffffffffu, careful[0] || careful[1]);
     float s[kKeys / 8][4];
 #pragma unroll
     for (int n = 0; n < kKeys / 8; ++n)
@@ -308,7 +307,7 @@ __device__ __forceinline__ void take_keys(Running<D>& run, const uint32_t (&q)[D
             w[2 * j] = pack_weights<T>(x[0], x[1]);
             w[2 * j + 1] = pack_weights<T>(x[2], x[3]);
         }
-        if (any_careful) {
+        if (careful) {
             if constexpr (!kAscending) {           // the other entries as ever: their sums do not hang on their neighbours
 #pragma unroll
                 for (int d = 0; d < D / 16; ++d) {
@@ -321,7 +320,7 @@ __device__ __forceinline__ void take_keys(Running<D>& run, const uint32_t (&q)[D
                         mma16816<T>(sum, w, b[2 * j], b[2 * j + 1]);
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            if (!careful[i >> 1]) acc[i] = sum[i];
+                            if (!cut[i >> 1]) acc[i] = sum[i];
                     }
                 }
             }
@@ -332,7 +331,7 @@ __device__ __forceinline__ void take_keys(Running<D>& run, const uint32_t (&q)[D
                                           __shfl_sync(0xffffffffu, k < 8 ? w[1] : w[3], owner)};
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    if (!careful[i] || key < low[i] || key >= high[i]) continue;
+                    if (!cut[i] || key < low[i] || key >= high[i]) continue;
                     const float2 pair = unpack2<T>(both[i]);
                     const float weight = (k & 1) ? pair.y : pair.x;
 #pragma unroll
@@ -451,8 +450,8 @@ __global__ void __launch_bounds__(kBpThreads) block_attention_tiles_kernel(const
             }
             const int left = cached - o;
             const int low[2] = {0, 0}, high[2] = {min(before[0] - o, left), min(before[1] - o, left)};
-            const bool careful[2] = {before[0] < cached && !finite, before[1] < cached && !finite};
-            take_keys<T, D, kKeys, false>(run, q, keys, values, low, high, a.scale_log2, careful, staged_values);
+            const bool cut[2] = {before[0] < cached, before[1] < cached};
+            take_keys<T, D, kKeys, false>(run, q, keys, values, low, high, a.scale_log2, clipped && !finite, cut, staged_values);
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -574,8 +573,7 @@ __global__ void __launch_bounds__(kTtRows, D == 64 ? 6 : 3) block_attention_tens
         }
         cp_async_commit();
         const int2 mine = entries[first + tid];
-        auto seen = [&](int pair) { return pair < 0 ? cached : min(max(g.t0 + (pair >> kBpRankBits) - a.window + 1, 0) - at, cached); };
-        const int before = seen(mine.x);
+        const int before = mine.x < 0 ? cached : min(max(g.t0 + (mine.x >> kBpRankBits) - a.window + 1, 0) - at, cached);
         cp_async_wait_all();
         fence_proxy_async();
         const bool clipped = __syncthreads_or(before < cached);
@@ -635,8 +633,6 @@ __global__ void __launch_bounds__(kTtRows, D == 64 ? 6 : 3) block_attention_tens
         const float base = top == kNegInf ? 0.0f : top;
         float2 sum2 = make_float2(0.0f, 0.0f);
         const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), base2 = make_float2(-base, -base);
-        // an entry's own matter, so that its sums do not hang on its neighbours
-        auto careful = [&](int pair) { return !finite && seen(pair) < cached; };
 #pragma unroll
         for (int c = 0; c < kKeys / 16; ++c) {
             float x[16];
@@ -662,8 +658,10 @@ __global__ void __launch_bounds__(kTtRows, D == 64 ? 6 : 3) block_attention_tens
             const int row = mine.x >> kBpRankBits, rank = mine.x & ((1 << kBpRankBits) - 1);
             const int64_t entry = ((static_cast<int64_t>(row) * a.kv_heads + kv) * a.top + rank) * a.group + mine.y;
             reinterpret_cast<float2*>(g.base + p.plan.stats)[entry] = make_float2(top, sum2.x + sum2.y);
-            if (careful(mine.x)) {
-                // the weighted sum on the CUDA cores, of the keys that the entry sees, 16 components at a time
+            if (!finite && before < cached) {
+                // the weighted sum on the CUDA cores, of the keys that the entry sees, 16 components at a time: the entry's own
+                // matter, so that its neighbours' sums do not hang on it; below, its place is passed by
+                entries[first + tid].x = -1;
                 float* sums = reinterpret_cast<float*>(g.base + p.plan.sums) + entry * D;
 #pragma unroll 1
                 for (int d = 0; d < D; d += 16) {
@@ -714,7 +712,7 @@ __global__ void __launch_bounds__(kTtRows, D == 64 ? 6 : 3) block_attention_tens
                 const int2 other = entries[first + 32 * warp + 16 * half + (lane >> 2) + 8 * i];
                 const int row = other.x >> kBpRankBits, rank = other.x & ((1 << kBpRankBits) - 1);
                 const int64_t entry = ((static_cast<int64_t>(row) * a.kv_heads + kv) * a.top + rank) * a.group + other.y;
-                to[i] = other.x < 0 || careful(other.x) ? nullptr : reinterpret_cast<float*>(g.base + p.plan.sums) + entry * D + 4 * (lane & 3);
+                to[i] = other.x < 0 ? nullptr : reinterpret_cast<float*>(g.base + p.plan.sums) + entry * D + 4 * (lane & 3);
             }
 #pragma unroll
             for (int b = 0; b < D / 64; ++b) {
@@ -827,14 +825,13 @@ __global__ void __launch_bounds__(kBpThreads, D <= 64 ? 4 : 2) block_attention_w
             const unsigned char* staged_values = memory + kBpEntries * S::kRowBytes + stage * kStage + kKeys * S::kRowBytes;
             // keys that every row of the tile sees may hold anything
             const bool all = at >= g.t0 + last_q + 1 - a.window && at + kKeys <= g.t0 + first_q + 1;
-            const bool not_finite = !all && __syncthreads_or(staged_not_finite<T, D, kKeys>(staged_values, threadIdx.x, kBpThreads));
-            const bool careful[2] = {not_finite, not_finite};
+            const bool careful = !all && __syncthreads_or(staged_not_finite<T, D, kKeys>(staged_values, threadIdx.x, kBpThreads));
             if (round == 0) load_queries<D>(q, staged_q + 16 * warp * S::kRowBytes, a.flip);
             const int low[2] = {from[0] - at, from[1] - at}, high[2] = {to[0] - at, to[1] - at};
             // a warp none of whose rows sees these keys passes
             if (__any_sync(0xffffffffu, high[1] > 0 && low[0] < kKeys))
                 take_keys<T, D, kKeys, true>(run, q, ring + stage * kStage, ring + stage * kStage + kKeys * S::kRowBytes, low, high,
-                                             a.scale_log2, careful, staged_values);
+                                             a.scale_log2, careful, {true, true}, staged_values);
             __syncthreads();
             stage ^= 1;
         }
