@@ -810,7 +810,8 @@ int rlm_block_route(const void* router_query, int64_t query_row_stride, const vo
  * of the blocks in block_index [n_rows, kv_heads, top_blocks]: [n * block_size, min((n + 1) * block_size, ls)).  Negative
  * indices and repeated ones count for nothing.  Query head h reads key head h / (heads / kv_heads).  out [n_rows, heads,
  * width] in the operands' dtype, lse [n_rows, heads] fp32, the natural logarithm of the softmax denominator.  Sums,
- * maxima and logarithms in fp32; 16-bit operands multiply on the tensor cores, their weights rounded to 16 bits.
+ * maxima and logarithms in fp32; 16-bit operands multiply on the tensor cores, their weights rounded to 16 bits (fp16:
+ * carried 2^15-fold, all bits down to 2^-29 of the largest).  Strides of dimensions of one are not looked at.
  * `strides`: 10 HOST int64, in elements: query row, head; key cache sequence, row, head; value cache sequence, row, head;
  * block_index row, head.  Widths 32, 64, 96, 128.
  */

@@ -17,9 +17,10 @@
 // The tiles of head widths 64 and 128 and blocks of up to 64 keys multiply on tcgen05; other widths and blocks, and the windows,
 // whose keys differ from row to row, on the warp-level instruction, 16 entries a warp, operands in registers from the scores to
 // the weighted sum.  What bounds the passes is the partial results' bytes, 8 D bytes an entry and block written and read, and
-// the chain of steps of a tile.  8 x 4096 rows, 8 heads over 2 of width 64, four blocks of 64: 175 us, of which the sort 9, the
-// tiles 88 (69 without their stores), the windows 84 (the join alone 67, 268 MB at 4.0 TB/s; the windows alone 52; one after the
-// other in a CTA 92); row by row 1471.
+// the chain of steps of a tile.  8 x 4096 rows, 8 heads over 2 of width 64, four blocks of 64: 174 us, row by row 1471.  Each pass
+// for itself under a profiler (its 185 are more than the 174 of the passes in a row): sort 11, tiles 89, windows 85.  In working
+// copies the tiles without their stores took 69 us, the join alone 67 (268 MB of partial results, 4.0 TB/s), the windows alone 52,
+// windows and join one after the other in a CTA 92.
 #include "block_attention_mma.cuh"
 #include "rlm_tcgen05.cuh"
 

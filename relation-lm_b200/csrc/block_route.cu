@@ -12,7 +12,7 @@
 //
 // Bytes bound long caches (256 bytes a block and row in 16 bits), latency the short ones.  Eight lanes share a block,
 // 16 bytes of its mean and of its spread each, so a warp's load covers four whole rows of a statistic.  One row of 16 blocks
-// 4.1 us, of 1024 blocks (over eight CTAs) 10.9; 256 rows of 1024 blocks 20 us from L2 (3.3 TB/s), 23.5 at unequal lengths
+// 4.1 to 4.5 us, of 1024 blocks (over eight CTAs) 10.9; 256 rows of 1024 blocks 20 us from L2 (3.3 TB/s), 23.7 at unequal lengths
 // from memory, a CTA a row.
 #include "block_attention_mma.cuh"
 
@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(kBrThreads, kDeep ? 2 : 4) block_route_kernel(
         if (lane == 0) atomicMax(&slack_of[own_row], widest);
         row_sync();
         const float slack = slack_of_size(__uint_as_float(slack_of[own_row]));
-        // a threshold that TOP blocks reach: the TOP-th largest of the largest of 4 TOP or more groups of blocks
+        // a threshold that TOP blocks reach: the TOP-th largest of the largest of 2 TOP or more groups of blocks
         if (a.top <= kRowThreads && a.top < able) {
             int groups = kRowThreads, of = 1;            // of consecutive threads share a group, every groups-th block
             while (of < 32 && groups >= 8 * a.top && groups > 32) {

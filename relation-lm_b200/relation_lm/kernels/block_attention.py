@@ -44,7 +44,9 @@ def rotary_frequencies(rotary: int, base: float = 10000.0, *, scaling: str | Non
     ``scaling`` stretches them for contexts ``factor`` times the trained one: ``"linear"`` divides them by ``factor``;
     ``"base"`` raises the base so that the slowest is divided by ``factor`` and the fastest stays; ``"by_parts"`` (Peng et
     al., YaRN, 2023) divides those that turn fewer than ``slow`` times in ``trained_context`` positions, leaves those that
-    turn more than ``fast`` times, blends in between, and returns the magnitude ``1 + 0.1 log(factor)``.
+    turn more than ``fast`` times, blends in between, and returns the magnitude ``1 + 0.1 log(factor)``.  The blend is linear
+    in the number of turns, as published; models trained with one that is linear in the component's index ``i`` need their own
+    frequencies, which ``rotary_append`` takes as they are.
     """
     if rotary < 0 or rotary % 2 != 0:
         raise ValueError("the rotary width must be even")
@@ -171,7 +173,8 @@ def block_attention(query: Tensor, key_cache: Tensor, value_cache: Tensor, block
     for all heads, or ``[N, kv_heads, blocks]``; negative and repeated indices count for nothing, at most 128 are given.
     Query head ``h`` reads key head ``h // (heads / kv_heads)`` of the caches ``[B, T, kv_heads, width]`` (any strides but the
     innermost; widths 32, 64, 96, 128; rows on 16-byte boundaries).  ``lse`` (fp32) is the logarithm of the softmax denominator; a row that sees
-    nothing is zero with -inf.  Sums are fp32, 16-bit operands' softmax weights are rounded to 16 bits.
+    nothing is zero with -inf.  Sums are fp32, 16-bit operands' softmax weights are rounded to 16 bits (half a step of each weight;
+    in fp16 all bits down to 2^-29 of the row's largest).  A block may be longer than the cache.
     """
     return _block_attention(query, key_cache, value_cache, block_index, position, block_size, local_window, scale)
 
@@ -199,7 +202,11 @@ def _(query, key_cache, value_cache, block_index, row_batch, row_position, block
 
 def block_attention_prefill(query: Tensor, key_cache: Tensor, value_cache: Tensor, block_index: Tensor, query_length: int,
                             block_size: int, local_window: int, scale: float) -> tuple[Tensor, Tensor]:
-    """``block_attention`` for positions ``0 .. query_length - 1`` of every sequence."""
+    """``block_attention`` for positions ``0 .. query_length - 1`` of every sequence.
+
+    In 16 bits and from about a thousand (row, key head) pairs on it allocates a workspace for the duration of the call: about
+    ``4 * heads * blocks * (width + 2)`` bytes a row, up to some 512 MB (at least one part of a sequence), whatever the batch.
+    """
     return _block_attention_prefill(query, key_cache, value_cache, block_index, query_length, block_size, local_window, scale)
 
 
