@@ -97,6 +97,11 @@ __device__ __forceinline__ uint32_t load_pair(const void* p) { return __ldg(stat
 // that of the exponentials' sum and its logarithm below 2^-19; twice as much is allowed for.
 __device__ __forceinline__ float slack_of_size(float size) { return fmaf(size, 3.814697265625e-6f, 7.62939453125e-6f); }
 
+// Squares below 2^-149 vanish from a norm, sixteen of them at most 2^-145: norms begin at a little more.  With that the bounds
+// hold whatever the magnitudes, as long as the spreads' factor stays below kSteep; beyond it all blocks are scored in 64 bits.
+constexpr float kLeastNorm = 1e-43f;
+constexpr float kSteep = 1e10f;
+
 // Eight consecutive statistics as they lie in memory.
 template <typename T> struct RawStats;
 template <> struct RawStats<float> {
@@ -188,7 +193,7 @@ __global__ void __launch_bounds__(kBrThreads, kDeep ? 2 : 4) block_route_kernel(
 
     const double soft = soft_of[head];
     const float soft32 = static_cast<float>(soft);
-    float norm = 0.0f;                                   // of the query's head
+    float norm = soft32 <= kSteep ? kLeastNorm : INFINITY;           // of the query's head, squared
 #pragma unroll
     for (int i = 0; i < 8; ++i) norm = fmaf(q[i], q[i], norm);
     norm += __shfl_xor_sync(0xffffffffu, norm, 1);
@@ -228,7 +233,7 @@ __global__ void __launch_bounds__(kBrThreads, kDeep ? 2 : 4) block_route_kernel(
                 mean[u].widen(m);
                 spreadv[u].widen(s);
                 // magnitudes by Cauchy's inequality: |q . m| summed over magnitudes is at most |q| |m|
-                float near = 0.0f, near_norm = 0.0f, spread = 0.0f, spread_norm = 0.0f;
+                float near = 0.0f, near_norm = kLeastNorm, spread = 0.0f, spread_norm = kLeastNorm;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     near = fmaf(q[i], m[i], near);
@@ -425,7 +430,7 @@ __global__ void __launch_bounds__(kBtThreads, sizeof(T) == 4 ? 4 : 5) block_rout
                               load_scalar(a.bias, 2 * a.buckets + i, a.param_dtype), load_scalar(a.bias, 3 * a.buckets + i, a.param_dtype));
     if (threadIdx.x < 4) {
         soft_of[threadIdx.x] = soft_plus(load_scalar(a.gamma, threadIdx.x, a.param_dtype));
-        mean_norm[threadIdx.x] = spread_norm[threadIdx.x] = 0u;
+        mean_norm[threadIdx.x] = spread_norm[threadIdx.x] = __float_as_uint(kLeastNorm);
         float widest = 0.0f;
         for (int k = 0; k < a.buckets; ++k) {
             const float b = fabsf(load_scalar(a.bias, threadIdx.x * a.buckets + k, a.param_dtype));
@@ -467,7 +472,7 @@ __global__ void __launch_bounds__(kBtThreads, sizeof(T) == 4 ? 4 : 5) block_rout
         const T* row = static_cast<const T*>(a.query) + (first_row + (live ? t_of[i] : 0)) * a.q_stride;
 #pragma unroll
         for (int h = 0; h < 4; ++h) {
-            float n = 0.0f;
+            float n = kLeastNorm;
             if constexpr (sizeof(T) == 4) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
@@ -479,7 +484,7 @@ __global__ void __launch_bounds__(kBtThreads, sizeof(T) == 4 ? 4 : 5) block_rout
                 q[h][0][i] = load_pair(row + 16 * h + 2 * (lane & 3));
                 q[h][0][2 + i] = load_pair(row + 16 * h + 8 + 2 * (lane & 3));
                 const float2 x = unpack2<T>(q[h][0][i]), y = unpack2<T>(q[h][0][2 + i]);
-                n = x.x * x.x + x.y * x.y + y.x * y.x + y.y * y.y;
+                n += x.x * x.x + x.y * x.y + y.x * y.x + y.y * y.y;
             }
             n += __shfl_xor_sync(0xffffffffu, n, 1);
             n += __shfl_xor_sync(0xffffffffu, n, 2);
@@ -575,7 +580,8 @@ __global__ void __launch_bounds__(kBtThreads, sizeof(T) == 4 ? 4 : 5) block_rout
     // a row's slack: magnitudes by Cauchy's inequality from the norms; squares that overflow make everything a candidate
     bool wild = false;
 #pragma unroll
-    for (int h = 0; h < 4; ++h) wild = wild || !(__uint_as_float(mean_norm[h]) < 3.0e38f) || !(__uint_as_float(spread_norm[h]) < 3.0e38f);
+    for (int h = 0; h < 4; ++h)
+        wild = wild || !(__uint_as_float(mean_norm[h]) < 3.0e38f) || !(__uint_as_float(spread_norm[h]) < 3.0e38f) || !(soft[h] <= kSteep);
     float slack[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {

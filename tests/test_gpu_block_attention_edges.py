@@ -539,3 +539,31 @@ def test_whole_sequence_layer_by_the_three_passes(dtype):
                 within(y, want, bound, t)
                 within(z, want_lse, lse_bound, t)
     status_clear()
+
+
+@pytest.mark.parametrize("gamma,query,spread", [(1e22, 1e-23, 750.0), (1e25, 1e-12, 7.5e-11), (3e9, 1e-23, 2.0e16), (750.0, 1.0, 1.0)])
+@pytest.mark.parametrize("form", ("decode", "rows", "prefill"))
+def test_the_choice_is_that_of_64_bits_at_any_magnitude(form, gamma, query, spread):
+    # tiny queries under a steep factor: scores of hundreds whose magnitudes' squares vanish in 32 bits; blocks differ by the last
+    # bits of their spreads, less than what a score in 32 bits is off by
+    blocks, top = (1000, 9) if form != "prefill" else (120, 9)
+    g = torch.Generator().manual_seed(3)
+    step = torch.finfo(torch.float32).eps * 2.0 ** math.floor(math.log2(spread))
+    mean = torch.zeros(1, blocks, 4, 16)
+    std = (spread + torch.randint(0, 4, (1, blocks, 4, 16), generator=g).double() * step).float()
+    n = {"decode": 1, "rows": 600, "prefill": 9000}[form]
+    q = (query * (0.5 + 0.5 * torch.rand(n, 64, generator=g).double())).float()
+    at = plain.places(form, 1, 0, 0, n) if form == "prefill" else [(0, 4 * blocks - 1 - i) for i in range(n)]
+    size = 64 if form == "prefill" else 4
+    call = {"decode": ba.route_blocks, "rows": ba.route_blocks_rows, "prefill": ba.route_blocks_prefill}[form]
+    scales = torch.full((4,), gamma), torch.zeros(4, 1)
+    index, score = call(q.cuda(), mean.cuda(), std.cuda(), *[v.cuda() for v in scales], *plain.where(form, at, n), size, 0, top, False)
+    soft = float(scales[0][0].double())                  # softplus of factors this large, to less than 1e-300
+    for i in sorted({0, n // 3, n // 2, n - 2, n - 1}):
+        able = min((at[i][1] + 1) // size, blocks)
+        heads = soft * (q[i].double().view(4, 16) * std[0, :able].double()).sum(-1) / 4
+        value = torch.logsumexp(heads, 1)
+        want = sorted(range(able), key=lambda b: (-float(value[b]), b))[:top]
+        assert index[i].tolist() == want + [-1] * (top - len(want)), i
+        within(score[i][:len(want)], value[want], 2.0 ** -24 * value[want].abs() + 1e-12)
+    status_clear()
