@@ -760,6 +760,10 @@ int launch_route(RouteArgs& a, void* stream) {
                                           a.n_blocks / (2 * a.parts) >= 4 * a.top) ||
                                          kBrBytesPerBlock * (a.n_blocks / a.parts + 1) > kBrMemory))
             a.parts *= 2;
+        if (rows * a.parts > 0x7fffffff) {
+            set_error("block_route: too many rows of so many blocks for one launch");
+            return RLM_ERR_SHAPE;
+        }
         a.part_blocks = (a.n_blocks + a.parts - 1) / a.parts;
         const int bytes = kBrBytesPerBlock * a.part_blocks;
         const bool deep = a.n_blocks >= 2048 || (a.part_blocks >= 512 && rows * a.parts <= 2 * sm_count());

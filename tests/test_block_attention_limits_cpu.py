@@ -6,7 +6,7 @@ import ctypes
 import pytest
 
 from relation_lm.kernels import _abi
-from test_block_attention_cpu import ATTENTION, refused, strides
+from test_block_attention_cpu import ATTENTION, ROUTE, refused, strides
 
 
 def accepted(**changes):
@@ -22,3 +22,10 @@ def test_the_step_of_a_single_one_is_of_no_account(which, ones):
     none = dict(n_rows=0, position=None, row_batch=1 << 20, row_position=1 << 20, strides=strides(*steps))
     refused("rlm_block_attention", ATTENTION, -4, **none)
     accepted(**none, **ones)
+
+
+def test_more_rows_than_a_launch_holds_are_refused():
+    # rows whose blocks need a cluster of eight CTAs each: the number of CTAs passes 32 bits
+    many = dict(position=None, row_batch=1 << 20, row_position=1 << 20, n_rows=0x7fffffff, n_blocks=40000, block=1)
+    refused("rlm_block_route", ROUTE, -2, **many)
+    refused("rlm_block_attention", ATTENTION, -2, position=None, row_batch=1 << 20, row_position=1 << 20, n_rows=0x7fffffff)
